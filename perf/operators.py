@@ -22,17 +22,13 @@ _TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 _BYTES = {"bf16": 2, "f16": 2, "f32": 4}
 
 
-_loaded = []
-
-
 def _ops():
-    """The framework's operators, imported by the first call."""
-    if not _loaded:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "ss-grpo_b200"))
-        from flashgrpo_b200 import ops
+    root = str(Path(__file__).resolve().parents[1] / "ss-grpo_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from flashgrpo_b200 import ops
 
-        _loaded.append(ops)
-    return _loaded[0]
+    return ops
 
 
 # --------------------------------------------------------------------- cases
