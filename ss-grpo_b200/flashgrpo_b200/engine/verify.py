@@ -332,7 +332,7 @@ class RoundBuffers:
         ws = ops.attention_workspace_bytes(B, N_, spec.n_q_heads, spec.n_kv_heads, spec.head_dim, num_splits=0,
                                            max_kv_len=0)
         self.ws_bytes = ws
-        self.attn_ws = None
+        self.attn_ws: dict = {}  # by capacity and splits
         self.logprobs: dict = {}  # of the accepted tokens, by the number of alternatives
 
 
@@ -447,12 +447,17 @@ class VerifyEngine:
         return ws
 
     def _attn_workspace(self, rb: RoundBuffers, st: DecodeState, splits: int):
-        need = (ops.kv8_attention_workspace_bytes if self.kv8 else ops.attention_workspace_bytes)(st.B, rb.N, self.spec.n_q_heads, self.spec.n_kv_heads,
-                                             self.spec.head_dim, num_splits=splits,
-                                             **{"max_q_len" if self.kv8 else "max_kv_len": st.capacity})
-        if need and (rb.attn_ws is None or rb.attn_ws.numel() * 4 < need):
-            rb.attn_ws = torch.zeros(need // 4 + 64, dtype=torch.int32, device=self.device)
-        return rb.attn_ws
+        """The tree attention's workspace for this capacity and split choice
+        (None when it needs none).  Each has its own, which stays: captured
+        rounds hold its address, and the kernels' layout of it (partials, then
+        counters that have to be zero) depends on the split plan."""
+        sp, key = self.spec, (st.capacity, splits)
+        if key not in rb.attn_ws:
+            size, most = ((ops.kv8_attention_workspace_bytes, "max_q_len") if self.kv8 else
+                          (ops.attention_workspace_bytes, "max_kv_len"))
+            need = size(st.B, rb.N, sp.n_q_heads, sp.n_kv_heads, sp.head_dim, num_splits=splits, **{most: st.capacity})
+            rb.attn_ws[key] = (torch.zeros(need // 4 + 64, dtype=torch.int32, device=self.device) if need else None)
+        return rb.attn_ws[key]
 
     def _native_dense(self, cfg: RoundConfig) -> bool:
         """fg_linear can run this model's projections (bf16, K multiples of 64)

@@ -1,0 +1,74 @@
+"""generate() in the calls that follow one another on a decoder: several
+lengths, with both caches."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import cuda_available
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not cuda_available(), reason="needs a CUDA device")]
+
+
+class _Tok:
+    pad_token_id = 0
+    eos_token_id = 1
+
+
+@pytest.fixture(scope="module")
+def bf16_model():
+    """Two layers of the 1.5B shape: head_dim 128, the tensor-core kernels."""
+    from flashgrpo_b200.utils import synthetic
+
+    return synthetic.build_model(2, layers=2, vocab=4096).cuda()
+
+
+def bf16_heads(n=3):
+    g = torch.Generator().manual_seed(0)
+    heads = {}
+    for i in range(n):
+        heads[f"heads.{i}.norm.weight"] = torch.ones(1536).bfloat16().cuda()
+        heads[f"heads.{i}.norm.bias"] = torch.zeros(1536).bfloat16().cuda()
+        heads[f"heads.{i}.fc.weight"] = (torch.randn(1536, 1536, generator=g) * 0.02).bfloat16().cuda()
+        heads[f"heads.{i}.fc.bias"] = torch.zeros(1536).bfloat16().cuda()
+    return heads
+
+
+def bf16_decoder(model, **kw):
+    from flashgrpo_b200.decoding.flash_medusa_decoder import FlashMedusaConfig, FlashMedusaDecoder
+
+    cfg = dict(tree_mode="fixed", max_tree_nodes_per_seq=13, max_tree_depth=4, fixed_tree_topk_by_depth=(4, 2),
+               top_p=1.0, sampling_seed=7, autotune_dense=False)
+    return FlashMedusaDecoder(model, bf16_heads(), _Tok(), FlashMedusaConfig(**{**cfg, **kw}))
+
+
+@pytest.mark.parametrize("cache", ["model", "fp8"])
+def test_one_decoder_with_two_capacities(bf16_model, cache):
+    """Short, long, short: the long call's split plan needs a larger workspace of another layout on the same round
+    buffers, and the captured rounds of the short one are replayed behind it.  Every call gives the tokens of its first
+    run and of eager rounds (the same kernels with the same plans: the same bits)."""
+    from flashgrpo_b200 import _native, ops
+    from flashgrpo_b200.utils import synthetic
+
+    kw = dict(kv_cache_dtype=cache, return_logprobs=True)
+    size = ops.kv8_attention_workspace_bytes if cache == "fp8" else ops.attention_workspace_bytes
+    most = "max_q_len" if cache == "fp8" else "max_kv_len"
+    calls = [(500, 524), (2500, 2524)]
+    need = [size(2, 13, 12, 2, 128, num_splits=0, **{most: m + 15}) for _, m in calls]
+    assert 0 < need[0] < need[1]
+    dec = bf16_decoder(bf16_model, **kw)
+    got = []
+    for which in (0, 0, 1, 1, 0, 1, 0):
+        n, most_len = calls[which]
+        ids, mask = synthetic.random_prompts(1, n, 4096, seed=3)
+        r = dec.generate(ids, mask, repeated_generate_nums=2, max_length=most_len)
+        got.append((which, r["generated_token_ids"], r["generated_logprobs"]))
+    for which in (0, 1):
+        n, most_len = calls[which]
+        ids, mask = synthetic.random_prompts(1, n, 4096, seed=3)
+        r = bf16_decoder(bf16_model, use_cuda_graphs=False, **kw).generate(ids, mask, repeated_generate_nums=2,
+                                                                           max_length=most_len)
+        for w, toks, lps in got:
+            if w == which:
+                assert toks == r["generated_token_ids"] and lps == r["generated_logprobs"]
+    assert _native.read_device_error(clear=True) == 0
