@@ -438,13 +438,17 @@ class VerifyEngine:
         return (cfg.lm_head == "fused" and sp.dtype == torch.bfloat16 and sp.hidden % 64 == 0 and M <= 256
                 and self.w.lm_head.stride(1) == 1)
 
+    def _grown_ws(self, name: str, need: int) -> torch.Tensor:
+        """A workspace of `need` bytes that calls of one kind share, the last
+        of those made so far if that is large enough.  One that a larger call
+        replaces stays allocated: captured rounds hold its address."""
+        made = self._graphs.setdefault(("ws", name), [])
+        if not made or made[-1].numel() * 4 < need:
+            made.append(torch.empty(max(need, 16) // 4 + 64, dtype=torch.int32, device=self.device))
+        return made[-1]
+
     def _lm_head_ws(self, M: int, topk_row0: int, k: int) -> torch.Tensor:
-        need = ops.lm_head_topk_workspace_bytes(M, self.spec.vocab, topk_row0, k)
-        ws = getattr(self, "_lmh_ws", None)
-        if ws is None or ws.numel() * 4 < need:
-            ws = torch.empty(max(need, 16) // 4 + 64, dtype=torch.int32, device=self.device)
-            self._lmh_ws = ws
-        return ws
+        return self._grown_ws("lm_head", ops.lm_head_topk_workspace_bytes(M, self.spec.vocab, topk_row0, k))
 
     def _attn_workspace(self, rb: RoundBuffers, st: DecodeState, splits: int):
         """The tree attention's workspace for this capacity and split choice
@@ -631,12 +635,8 @@ class VerifyEngine:
         self._linear_ws(rb.hid_int.shape[0], sp.vocab, sp.hidden, ops.EPI_STORE)
 
     def _propose_ws(self, B: int, nh: int, k: int) -> torch.Tensor:
-        need = ops.medusa_propose_workspace_bytes(B, self.spec.hidden, self.spec.vocab, nh, k)
-        ws = getattr(self, "_prop_ws", None)
-        if ws is None or ws.numel() * 4 < need:
-            ws = torch.empty(max(need, 16) // 4 + 64, dtype=torch.int32, device=self.device)
-            self._prop_ws = ws
-        return ws
+        return self._grown_ws("propose", ops.medusa_propose_workspace_bytes(B, self.spec.hidden, self.spec.vocab, nh,
+                                                                            k))
 
     def propose(self, st: DecodeState, rb: RoundBuffers, cfg: RoundConfig):
         B, nh = st.B, rb.n_heads
@@ -699,13 +699,8 @@ class VerifyEngine:
 
     def _chain_ws(self, M: int, k: int) -> torch.Tensor:
         sp = self.spec
-        need = ops.chain_step_workspace_bytes(M, sp.hidden, self.heads.chain["state_proj.weight"].shape[0],
-                                              sp.vocab, k)
-        ws = getattr(self, "_chain_ws_buf", None)
-        if ws is None or ws.numel() * 4 < need:
-            ws = torch.empty(max(need, 16) // 4 + 64, dtype=torch.int32, device=self.device)
-            self._chain_ws_buf = ws
-        return ws
+        return self._grown_ws("chain", ops.chain_step_workspace_bytes(
+            M, sp.hidden, self.heads.chain["state_proj.weight"].shape[0], sp.vocab, k))
 
     def _chain_topk_bufs(self, M: int, k: int):
         return (torch.empty((M, k), dtype=torch.int32, device=self.device),

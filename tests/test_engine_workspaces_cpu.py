@@ -42,3 +42,23 @@ def test_attention_workspaces_of_two_capacities(kv8):
     c = e._attn_workspace(rb, small, 3)
     assert c.data_ptr() not in (at, b.data_ptr()) and not c.any()
     assert e._attn_workspace(rb, large, 1) is None
+
+
+@pytest.mark.parametrize("call", [lambda e, big: e._lm_head_ws(200 if big else 8, 0, 4),
+                                  lambda e, big: e._propose_ws(64 if big else 2, 3, 4),
+                                  lambda e, big: e._chain_ws(200 if big else 8, 4)],
+                         ids=["lm_head", "propose", "chain"])
+def test_a_replaced_workspace_stays(call):
+    """A larger batch takes a new workspace; the one that captured rounds of the smaller batch hold is not freed (a
+    weak reference to it lives) and serves no other tensor."""
+    import weakref
+
+    e = engine(False)
+    e.heads = SimpleNamespace(chain={"state_proj.weight": torch.empty(256, 1536)})
+    small = call(e, False)
+    at, ref = small.data_ptr(), weakref.ref(small)
+    del small
+    large = call(e, True)
+    assert large.data_ptr() != at and large.numel() > ref().numel()
+    assert ref() is not None and ref().data_ptr() == at
+    assert call(e, True) is large
