@@ -155,7 +155,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, rows: torch.Te
     k = int(k)
     if out is None:
         f = dict(dtype=torch.float32, device=logits.device)
-        out = TokenLogprobs(*torch.empty((3, n), **f).unbind(0),
+        # tensors of their own: callers change them in place
+        out = TokenLogprobs(*[torch.empty(n, **f) for _ in range(3)],
                             torch.empty((n, k), dtype=torch.int32, device=logits.device) if k else None,
                             torch.empty((n, k), **f) if k else None)
     else:

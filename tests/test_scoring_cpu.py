@@ -1,0 +1,92 @@
+"""The differentiable log probabilities on the CPU: the launches are replaced by
+the formulas, what is tested is what lies around them (autograd, refusals)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def scoring(monkeypatch):
+    """engine.scoring with fg_token_logprobs and its gradient computed by torch on the CPU, into the tensors that the
+    wrappers pass."""
+    from flashgrpo_b200 import ops
+    from flashgrpo_b200.engine import scoring as s
+
+    known = {}  # address -> tensor: the stand-in of a launch sees pointers alone
+
+    def ptr(t):
+        if t is None:
+            return None
+        known[t.data_ptr()] = t
+        return t.data_ptr()
+
+    def call(t, name, *a, **kw):
+        get = lambda p: None if p is None else known[p]  # noqa: E731
+        if name == "fg_token_logprobs":
+            logits, tok, T = get(a[0]), get(a[6]), a[8]
+            logp, ent, lse = map(get, a[9:12])
+            n = tok.numel()
+            x = logits[:n].detach().float() / T
+            z = torch.log_softmax(x, 1)
+            live = tok >= 0
+            zero = torch.zeros(())
+            logp.copy_(torch.where(live, z.gather(1, tok.clamp(min=0).long()[:, None])[:, 0], zero))
+            ent.copy_(torch.where(live, -(z.exp() * z).sum(1), zero))
+            lse.copy_(torch.where(live, torch.logsumexp(x, 1), zero))
+        else:
+            assert name == "fg_token_logprobs_backward"
+            logits, tok, n, T = get(a[0]), get(a[4]), a[5], a[6]
+            lse, ent, g, h, out = map(get, a[7:12])
+            z = logits[:n].detach().float() / T - lse[:, None]
+            one = torch.zeros_like(z).scatter_(1, tok.clamp(min=0).long()[:, None], 1.0)
+            d = g[:, None] * (one - z.exp())
+            if h is not None:
+                d = d - h[:, None] * z.exp() * (z + ent[:, None])
+            out[:n].copy_((d / T).masked_fill((tok < 0)[:, None], 0.0))
+
+    monkeypatch.setattr(ops, "_ptr", ptr)
+    monkeypatch.setattr(ops, "_call", call)
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+    monkeypatch.setattr(ops, "_need", lambda t, name, dtype=None, contiguous=True: None)
+    return s
+
+
+def plain(logits, tok, T=1.0):
+    z = torch.log_softmax(logits / T, -1)
+    live = tok >= 0
+    lp = z.gather(1, tok.clamp(min=0).long()[:, None])[:, 0]
+    return torch.where(live, lp, torch.zeros(())), torch.where(live, -(z.exp() * z).sum(1), torch.zeros(()))
+
+
+def case(n=7, V=31):
+    g = torch.Generator().manual_seed(1)
+    tok = torch.randint(0, V, (n,), generator=g, dtype=torch.int32)
+    tok[2] = -1
+    return torch.randn(n, V, generator=g).requires_grad_(), tok, torch.randn(n, generator=g)
+
+
+@pytest.mark.parametrize("change", [lambda lp, w: lp.mul_(w), lambda lp, w: lp.__setitem__(w > 0, 0.0),
+                                    lambda lp, w: lp.detach().zero_()], ids=["mul_", "setitem", "detached"])
+def test_log_probabilities_can_be_changed_in_place(scoring, change):
+    """What a trainer does to them behind the call (a mask, a weight); the entropy stays usable.  fp32 sums of 31 terms
+    on both sides."""
+    logits, tok, w = case()
+    lp, ent = scoring.token_logprobs(logits, tok)
+    change(lp, w)
+    (lp.sum() + (w * ent).sum()).backward()
+    x = logits.detach().clone().requires_grad_()
+    lp2, ent2 = plain(x, tok)
+    lp2 = lp2.clone()
+    change(lp2, w)
+    (lp2.sum() + (w * ent2).sum()).backward()
+    assert (logits.grad - x.grad).abs().max() < 64 * 2.0 ** -24 * 8
+
+
+def test_outputs_are_tensors_of_their_own(scoring):
+    from flashgrpo_b200 import ops
+
+    logits, tok, _ = case()
+    r = ops.token_logprobs(logits.detach(), tok)
+    assert all(t._base is None for t in (r.logp, r.entropy, r.lse))
+    assert len({t.untyped_storage().data_ptr() for t in (r.logp, r.entropy, r.lse)}) == 3
