@@ -19,7 +19,8 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature):
         r = ops.token_logprobs(logits, tokens, temperature=temperature)
-        ctx.save_for_backward(logits, tokens, r.lse, r.entropy)
+        # (the entropy is an output, which the caller may change in place)
+        ctx.save_for_backward(logits, tokens, r.lse, r.entropy.clone())
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         return r.logp, r.entropy

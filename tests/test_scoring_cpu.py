@@ -90,3 +90,19 @@ def test_outputs_are_tensors_of_their_own(scoring):
     r = ops.token_logprobs(logits.detach(), tok)
     assert all(t._base is None for t in (r.logp, r.entropy, r.lse))
     assert len({t.untyped_storage().data_ptr() for t in (r.logp, r.entropy, r.lse)}) == 3
+
+
+@pytest.mark.parametrize("change", [lambda e, w: e.mul_(w), lambda e, w: e.__setitem__(w > 0, 0.0),
+                                    lambda e, w: e.detach().zero_()], ids=["mul_", "setitem", "detached"])
+def test_entropies_can_be_changed_in_place(scoring, change):
+    """The gradient reads the entropy of the forward, not what the caller made of it."""
+    logits, tok, w = case()
+    lp, ent = scoring.token_logprobs(logits, tok)
+    change(ent, w)
+    ((w * lp).sum() + ent.sum()).backward()
+    x = logits.detach().clone().requires_grad_()
+    lp2, ent2 = plain(x, tok)
+    ent2 = ent2.clone()
+    change(ent2, w)
+    ((w * lp2).sum() + ent2.sum()).backward()
+    assert (logits.grad - x.grad).abs().max() < 64 * 2.0 ** -24 * 8
