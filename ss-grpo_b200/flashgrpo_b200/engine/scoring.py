@@ -40,6 +40,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     """(log probability, entropy) f32 [n] of tokens (int32 [n], negative:
     padded, zeros) under softmax(logits / temperature), logits [n, vocab] with
     contiguous rows; differentiable with respect to the logits."""
+    if logits.shape[0] != tokens.shape[0]:  # the gradient has one row per token
+        raise ValueError("logits and tokens must have one row each per entry")
     return _TokenLogprobs.apply(logits, tokens, float(temperature))
 
 

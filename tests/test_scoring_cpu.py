@@ -106,3 +106,11 @@ def test_entropies_can_be_changed_in_place(scoring, change):
     change(ent2, w)
     ((w * lp2).sum() + ent2.sum()).backward()
     assert (logits.grad - x.grad).abs().max() < 64 * 2.0 ** -24 * 8
+
+
+def test_logits_rows_behind_the_tokens_are_refused(scoring):
+    """Their gradient would lack those rows, which autograd notices in the backward pass alone."""
+    logits, tok, _ = case()
+    for bad in (tok[:5], tok[:0]):
+        with pytest.raises(ValueError):
+            scoring.token_logprobs(logits, bad)
