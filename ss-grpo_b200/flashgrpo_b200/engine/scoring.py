@@ -2,14 +2,18 @@
 policy-update side of the log probabilities that `generate(return_logprobs)`
 reports (the reference trainer's log-softmax + gather over rollout tokens).
 
-The logits of a chunk of positions are the only [positions, vocab] tensor: log
-probability, entropy and their gradient are fg_token_logprobs /
-fg_token_logprobs_backward on it.
+Log probability, entropy and their gradient are fg_token_logprobs /
+fg_token_logprobs_backward on the logits of a chunk of positions.  No more than
+one chunk's logits are kept: where there are several, each is made again in its
+backward pass (and its gradient, of the same size, lives with it).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
+from torch.utils.checkpoint import checkpoint
 
 from .. import ops
 from .verify import unwrap_causal_lm
@@ -50,7 +54,8 @@ def sequence_logprobs(causal_lm, input_ids: torch.Tensor, attention_mask: torch.
     """(log probability, entropy) f32 [B, S - prompt_len] of the tokens from
     position prompt_len on (at least 1), each given the tokens before it;
     zeros at positions with attention_mask 0.  Differentiable; `chunk`
-    positions' logits are made at a time."""
+    positions' logits are made and kept at a time (in training the lm_head of
+    more than one chunk runs twice)."""
     B, S = input_ids.shape
     if not 1 <= prompt_len < S:
         raise ValueError("prompt_len must leave at least one token on each side")
@@ -64,7 +69,13 @@ def sequence_logprobs(causal_lm, input_ids: torch.Tensor, attention_mask: torch.
                         return_dict=True).last_hidden_state
     hidden = hidden[:, prompt_len - 1:S - 1].reshape(-1, hidden.shape[-1])
     tokens = torch.where(mask > 0, ids, -1)[:, prompt_len:].reshape(-1).to(torch.int32)
-    out = [token_logprobs(base.lm_head(hidden[a:a + chunk]), tokens[a:a + chunk].contiguous(),
-                          temperature=temperature) for a in range(0, hidden.shape[0], int(chunk))]
+
+    def score(h, t):
+        return _TokenLogprobs.apply(base.lm_head(h), t, float(temperature))
+
+    n, chunk = hidden.shape[0], int(chunk)
+    if torch.is_grad_enabled() and n > chunk:
+        score = functools.partial(checkpoint, score, use_reentrant=False)
+    out = [score(hidden[a:a + chunk], tokens[a:a + chunk].contiguous()) for a in range(0, n, chunk)]
     logp, entropy = (torch.cat(x).view(B, S - prompt_len) for x in zip(*out))
     return logp, entropy

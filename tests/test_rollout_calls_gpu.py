@@ -72,3 +72,29 @@ def test_one_decoder_with_two_capacities(bf16_model, cache):
             if w == which:
                 assert toks == r["generated_token_ids"] and lps == r["generated_logprobs"]
     assert _native.read_device_error(clear=True) == 0
+
+
+def test_sequence_logprobs_memory_goes_by_the_chunk():
+    """What a forward leaves on the device, and the peak of the backward behind it: of 4096 positions and a vocabulary
+    of 4096 in fp32 (64 MB of logits) the chunks of 256 (4 MB, twice with the gradient) keep no more than one."""
+    from flashgrpo_b200.engine.scoring import sequence_logprobs
+    from flashgrpo_b200.utils import synthetic
+
+    m = synthetic.build_model(1).cuda()
+    m.lm_head.weight.requires_grad_(True)
+    ids = torch.randint(0, 4096, (16, 264), generator=torch.Generator().manual_seed(5)).cuda()
+    mask = torch.ones_like(ids)
+    held, peak, grads = {}, {}, {}
+    for chunk in (256, 4096, 256):
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        lp, ent = sequence_logprobs(m, ids, mask, prompt_len=8, chunk=chunk)
+        held[chunk] = torch.cuda.memory_allocated() - start
+        torch.cuda.reset_peak_memory_stats()
+        grads[chunk], = torch.autograd.grad(lp.sum() + 0.1 * ent.sum(), m.lm_head.weight)
+        peak[chunk] = torch.cuda.max_memory_allocated() - start
+        del lp, ent
+    mb = 1 << 20
+    assert held[256] + 56 * mb < held[4096], held
+    assert peak[256] < held[256] + 32 * mb < peak[4096], (held, peak)
+    assert (grads[256] - grads[4096]).norm() <= 2.5e-4 * grads[4096].norm()

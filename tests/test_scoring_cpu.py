@@ -114,3 +114,47 @@ def test_logits_rows_behind_the_tokens_are_refused(scoring):
     for bad in (tok[:5], tok[:0]):
         with pytest.raises(ValueError):
             scoring.token_logprobs(logits, bad)
+
+
+@pytest.fixture(scope="module")
+def causal_lm():
+    from flashgrpo_b200.utils import synthetic
+
+    return synthetic.build_model(1)
+
+
+def sequences(B=3, S=20):
+    ids = torch.randint(0, 4096, (B, S), generator=torch.Generator().manual_seed(2))
+    mask = torch.ones_like(ids)
+    mask[1, :4] = 0
+    return ids, mask
+
+
+@pytest.mark.parametrize("chunk", [7, 1000])
+def test_sequence_logprobs_keep_one_chunk_of_logits(scoring, causal_lm, chunk):
+    """Between the forward and the backward pass no [positions, vocab] tensor of several chunks is saved, and the
+    gradient is that of the whole (fp32 sums over the vocabulary of 4096 and the positions in another order)."""
+    ids, mask = sequences()
+    w = causal_lm.lm_head.weight.requires_grad_(True)
+    saved = []
+    try:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(tuple(t.shape)) or t, lambda t: t):
+            lp, ent = scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5, chunk=chunk)
+        kept = [s for s in saved if len(s) == 2 and s[1] == 4096 and s[0] != 256]  # (256: the lm_head, transposed)
+        assert len(kept) == (1 if chunk >= 45 else 0), kept
+        got = torch.autograd.grad(lp.sum() + 0.3 * ent.sum(), w)[0]
+        pos = (mask.cumsum(-1) - 1).clamp(min=0)
+        logits = causal_lm(input_ids=ids, attention_mask=mask, position_ids=pos).logits[:, 4:-1].reshape(-1, 4096)
+        lp2, ent2 = plain(logits, torch.where(mask > 0, ids, -1)[:, 5:].reshape(-1).int())
+        want = torch.autograd.grad(lp2.sum() + 0.3 * ent2.sum(), w)[0]
+        assert (lp.reshape(-1) - lp2).abs().max() < 1e-4 and (got - want).norm() <= 2.5e-4 * want.norm()
+    finally:
+        causal_lm.lm_head.weight.requires_grad_(False)
+
+
+def test_sequence_logprobs_without_gradients(scoring, causal_lm):
+    ids, mask = sequences()
+    with torch.no_grad():
+        a = scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5, chunk=7)
+        b = scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
+    assert all((x - y).abs().max() < 1e-4 and not x.requires_grad for x, y in zip(a, b))
