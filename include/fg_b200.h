@@ -428,8 +428,10 @@ fg_status fg_kv8_commit(const fg_kv8_cache *cache, const int32_t *acc_nodes, int
  *   set; a node that attends to nothing gets zeros.
  * Scores, softmax statistics and sums are fp32; weights enter the product
  * with V as f16 with a power of two of their own (dtype bf16, head_dim 128) or
- * fp32.  No other slot is read; those read
- * must hold finite values (the tree slots also where no node sees them).
+ * fp32.  No other slot is read, and what a node does not see does not reach
+ * its rows, whatever it holds.  A NaN or an infinity in a query row, or in K
+ * or V of a tail slot that a node sees, gives NaN in the rows concerned (one
+ * in V an infinity where the kernel sums in fp32).
  * scale > 0 and finite.  max_q_len (a hint for the KV splits, >= 0): the
  * longest q_len of the batch; num_splits 0 = automatic, at most 64
  * (FG_EINVAL above).  workspace: fg_tree_attention_kv8_workspace_size bytes

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(128) attn_general_kernel(const AttnParams p) {
             }
         }
         float mx = -INFINITY;
+        uint32_t vis = 0;  // slots of the block that row r sees
 #pragma unroll
         for (int j = 0; j < kBlk / 4; ++j) {
             const int t = c + 4 * j;
@@ -132,9 +133,14 @@ __global__ void __launch_bounds__(128) attn_general_kernel(const AttnParams p) {
                 const int x = s0 + t - len.t;
                 see = (p.anc[node * 4 + (x >> 5)] >> (x & 31)) & 1u;
             }
-            s[j] = see ? s[j] * p.scale : -INFINITY;
+            vis |= (uint32_t)see << t;
+            // an infinite score becomes NaN: -inf is what a masked slot has
+            s[j] *= p.scale;
+            s[j] = see ? fmaf(s[j], 0.0f, s[j]) : -INFINITY;
             mx = fmaxf(mx, s[j]);
         }
+        vis |= __shfl_xor_sync(0xffffffffu, vis, 1);
+        vis |= __shfl_xor_sync(0xffffffffu, vis, 2);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mn = fmaxf(m, mx);
@@ -160,6 +166,7 @@ __global__ void __launch_bounds__(128) attn_general_kernel(const AttnParams p) {
             acc[i].w *= alpha;
         }
         for (int t = 0; t < live; ++t) {
+            if (!((vis >> t) & 1u)) continue;  // whatever V holds there
             const float e = ps[r * 33 + t];
 #pragma unroll
             for (int i = 0; i < kMaxD / 16; ++i) {

@@ -39,6 +39,8 @@
 // are numbered 0 .. q_len + tail_len + N - 1, tiles of 128 of them are read
 // with the last, mixed, ones first.  A tail row gets a power of two of its own
 // for K (hi + lo, like Q) and for V; slots past the end are zeros and masked.
+// A query row with a NaN or an infinity has scores of NaN, and so has a tail
+// slot whose K or V holds one, for the nodes that see it.
 // Every mbarrier wait is bounded as in fg_attention_tc.cu; after a timeout a
 // softmax warp runs on (so that the named barriers stay matched) and the CTA
 // writes nothing.
@@ -294,10 +296,11 @@ __device__ __forceinline__ uint32_t pair_mag(uint32_t w) {  // the larger magnit
     return max((w << 16) & 0x7fffffffu, w & 0x7fff0000u);
 }
 // 2^e that brings a largest magnitude (fp32 bits) times 2^-e into [2^7, 2^8);
-// 1 for zero, NaN and infinities.
+// 1 for zero, NaN for NaN and infinities (e4m3 and f16 would saturate those).
 __device__ __forceinline__ float fp8_scale_of(uint32_t mag) {
     const int ex = (int)(mag >> 23);
-    if (ex == 0 || ex == 255) return 1.0f;
+    if (ex == 0) return 1.0f;
+    if (ex == 255) return __int_as_float(0x7fffffff);
     return __uint_as_float((uint32_t)max(ex - 7, 1) << 23);
 }
 
@@ -437,7 +440,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_kv8_tc_kernel(const __grid
             const uint4 a = u[2 * s], c = u[2 * s + 1];
             if (is_v) {
                 uint4 lo, hi;
-                if (tail) {
+                if (tail && sc != sc) {
+                    // zeros: the slot's score becomes NaN instead, which
+                    // only the nodes that see it get
+                    lo = hi = make_uint4(0, 0, 0, 0);
+                } else if (tail) {
                     const float f = inv * 0x1p-8f;
                     lo = make_uint4(scale_even(a.x, a.y, f), scale_odd(a.x, a.y, f), scale_even(a.z, a.w, f),
                                     scale_odd(a.z, a.w, f));
@@ -745,6 +752,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_kv8_tc_kernel(const __grid
                 if (slot >= len.q && slot < T) {
                     kt = bars->tail_scale[0][i & 3][w4 * 32 + lane];
                     vt = bars->tail_scale[1][i & 3][w4 * 32 + lane];
+                    if (vt != vt) {  // V holds a NaN or an infinity
+                        kt = vt;
+                        vt = 1.0f;
+                    }
                 }
             }
             const float kc = kt * sc;

@@ -426,6 +426,37 @@ def test_attention_shows_a_poisoned_block(ops):
     assert out[1, :, :2].isnan().all() and out[1, :, 2:].isfinite().all() and out[2].isfinite().all()
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("what", ["q", "k_tail", "v_tail"])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 128)])
+def test_attention_shows_values_that_are_not_finite(ops, dtype, D, what, bad):
+    """One entry of a query row, of a tail token (all nodes see it) or of a tree node's K or V (its descendants and
+    itself do).  The rows that meet it show it, the others are what they are without it."""
+    lens = [100, 40, 5]
+    for splits in (1, 2):
+        cache, q, ql, tl, anc, scale = attention_case(ops, dtype, 3, 6, 4, 2, D, lens, 47)
+        want, tol = attention_reference(q, cache, 0, range(3), ql, tl, anc, scale)
+        bits = torch.tensor([[(int(w) >> j) & 1 for j in range(6)] for w in anc[:, 0].tolist()]).bool()
+        assert bits[:, 4].any() and not bits[:, 4].all()
+        hit = torch.zeros(3, 6, 4, dtype=torch.bool)  # rows that meet a bad value
+        if what == "q":
+            q[0, 2, 1, 7], q[2, 5, 3, D - 1] = bad, bad
+            hit[0, 2, 1] = hit[2, 5, 3] = True
+        else:
+            t = getattr(cache, what)
+            t[0, 0, 1, 2, 9] = bad             # a tail token of row 0, second KV head
+            t[0, 1, 0, int(tl[1]) + 4, D - 3] = bad  # node 4 of row 1, first KV head
+            hit[0, :, 2:] = True
+            hit[1, :, :2] = bits[:, 4:5]
+        hit = hit.to(DEV)
+        out = run_attention(ops, cache, q, ql, tl, anc, scale, splits=splits)
+        assert ((out.double() - want).abs() <= tol)[~hit].all()
+        if what == "v_tail" and not (dtype == torch.bfloat16 and D == 128):  # fp32 sums: in the dim it is in
+            assert not out[0, :, 2:, 9].isfinite().any() and not out[1][hit[1]][:, D - 3].isfinite().any()
+        else:
+            assert out[hit].isnan().all()
+
+
 def test_attention_bad_lengths_are_recorded(ops):
     from flashgrpo_b200 import _native as N
 
