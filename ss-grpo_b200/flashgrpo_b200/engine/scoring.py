@@ -40,12 +40,28 @@ class _TokenLogprobs(torch.autograd.Function):
         return ops.token_logprobs_backward(logits, tokens, lse, entropy, g, h, temperature=ctx.temperature), None, None
 
 
+def _check_ids(ids: torch.Tensor, least: int | None, end: int, name: str):
+    """Refuses ids outside [least, end): one host sync where they are on the
+    GPU, so not during a capture."""
+    if ids.is_cuda and torch.cuda.is_current_stream_capturing():
+        return
+    bad = ids >= end if least is None else (ids >= end) | (ids < least)
+    if bool(bad.any()):
+        raise ValueError(f"{name} must be below the vocabulary's {end} entries"
+                         + ("" if least is None else f" and at least {least}"))
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0):
     """(log probability, entropy) f32 [n] of tokens (int32 [n], negative:
     padded, zeros) under softmax(logits / temperature), logits [n, vocab] with
-    contiguous rows; differentiable with respect to the logits."""
+    contiguous rows; differentiable with respect to the logits.  A token
+    behind the vocabulary is refused (outside stream captures, in which it
+    gets zeros and sets the device error word)."""
     if logits.shape[0] != tokens.shape[0]:  # the gradient has one row per token
         raise ValueError("logits and tokens must have one row each per entry")
+    # the kernel would give such an entry zeros and record it in the device
+    # error word, which nobody reads here
+    _check_ids(tokens, None, logits.shape[-1], "tokens")
     return _TokenLogprobs.apply(logits, tokens, float(temperature))
 
 
@@ -55,13 +71,17 @@ def sequence_logprobs(causal_lm, input_ids: torch.Tensor, attention_mask: torch.
     position prompt_len on (at least 1), each given the tokens before it;
     zeros at positions with attention_mask 0.  Differentiable; `chunk`
     positions' logits are made and kept at a time (in training the lm_head of
-    more than one chunk runs twice)."""
+    more than one chunk runs twice).  Ids outside the embedding or the lm_head
+    are refused before anything runs."""
     B, S = input_ids.shape
     if not 1 <= prompt_len < S:
         raise ValueError("prompt_len must leave at least one token on each side")
     if attention_mask.shape != input_ids.shape:
         raise ValueError("attention_mask must have the shape of input_ids")
     base = unwrap_causal_lm(causal_lm)
+    _check_ids(input_ids, 0, base.model.get_input_embeddings().weight.shape[0], "input_ids")
+    _check_ids(torch.where(attention_mask.to(input_ids.device) > 0, input_ids, 0)[:, prompt_len:], 0, base.lm_head.weight.shape[0],
+               "scored input_ids")
     dev = base.lm_head.weight.device
     ids, mask = input_ids.to(dev), attention_mask.to(dev).long()
     pos = (mask.cumsum(-1) - 1).clamp(min=0)

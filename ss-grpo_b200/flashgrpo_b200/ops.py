@@ -143,7 +143,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, rows: torch.Te
     """Log probability of tokens[i] (int32 [n]; negative: a padded entry,
     which gets zeros) under softmax(logits[rows[i] or i] / temperature), the
     distribution's entropy and logsumexp, all f32 [n], and its k best entries
-    (top_idx int32, top_logp f32, [n, k]; value descending, index ascending)."""
+    (top_idx int32, top_logp f32, [n, k]; value descending, index ascending).
+    A token or row outside its range is treated as padded and sets the device
+    error word (_native.read_device_error)."""
     _need(logits, "logits", contiguous=False)
     stride, vocab = _rows(logits, "logits")
     n = _tokens(tokens, logits)
@@ -176,7 +178,8 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, lse: tor
                             temperature: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """d/dlogits of sum(grad_logp * logp + grad_entropy * entropy): [n, vocab]
     in the logits' dtype, with lse and entropy from token_logprobs (without
-    rows).  out may be the logits themselves (in place)."""
+    rows).  out may be the logits themselves (in place).  A token outside the
+    vocabulary gets zeros and sets the device error word."""
     _need(logits, "logits", contiguous=False)
     stride, vocab = _rows(logits, "logits")
     n = _tokens(tokens, logits)
@@ -516,7 +519,9 @@ def kv8_load(cache: Kv8Cache, layer: int, k: torch.Tensor, v: torch.Tensor, leng
              q_len: torch.Tensor, tail_len: torch.Tensor, *, repeats: int = 1) -> None:
     """fg_kv8_load: tokens [0, lengths[p]) of k / v [P, Hkv, S, D] (any
     strides, contiguous heads) to call rows p * repeats + j of one layer;
-    q_len / tail_len (int32 [P * repeats]) get the rows' lengths."""
+    q_len / tail_len (int32 [P * repeats]) get the rows' lengths.  A length
+    or mapped row that does not fit loads nothing and sets the device error
+    word (_native.read_device_error)."""
     for t, name in ((k, "k"), (v, "v")):
         _need(t, name, cache.dtype, contiguous=False)
         if t.dim() != 4 or t.shape[1] != cache.n_kv_heads or t.shape[3] != cache.head_dim:
@@ -540,7 +545,9 @@ def kv8_commit(cache: Kv8Cache, acc_nodes: torch.Tensor, acc_len: torch.Tensor, 
     """fg_kv8_commit: appends each row's accepted path (acc_nodes [B, dcap],
     acc_len [B], as accept_extract writes them) to its tail in every layer and
     quantises the completed blocks.  The new lengths go to q_len_out /
-    tail_len_out, or replace q_len / tail_len when those are omitted."""
+    tail_len_out, or replace q_len / tail_len when those are omitted.  A row
+    that does not fit the cache stays as it is and sets the device error
+    word."""
     _need(acc_nodes, "acc_nodes", torch.int32)
     _need(acc_len, "acc_len", torch.int32)
     B = acc_len.shape[0]
@@ -569,7 +576,8 @@ def tree_attention_kv8(q: torch.Tensor, cache: Kv8Cache, layer: int, q_len: torc
     """fg_tree_attention_kv8: q [B, N, Hq, D] over one layer of the cache; anc
     int32 [N, 4] bits.  max_q_len: the longest 8-bit prefix of the batch
     (default: the capacity), which the workspace (kv8_attention_workspace_bytes
-    for the same arguments) is sized for."""
+    for the same arguments) is sized for.  A length or mapped row outside the
+    cache is taken as an empty prefix and sets the device error word."""
     _need(q, "q", cache.dtype)
     if q.dim() != 4 or q.shape[3] != cache.head_dim or q.device != cache.device:
         raise ValueError("q must be [B, N, Hq, D] with the cache's head_dim, on its device")

@@ -158,3 +158,39 @@ def test_sequence_logprobs_without_gradients(scoring, causal_lm):
         a = scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5, chunk=7)
         b = scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
     assert all((x - y).abs().max() < 1e-4 and not x.requires_grad for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("bad", [31, 32, 1 << 30])
+def test_tokens_behind_the_vocabulary_are_refused(scoring, bad):
+    """The kernel would give such an entry log probability 0 and no gradient."""
+    logits, tok, _ = case()
+    tok[3] = bad
+    with pytest.raises(ValueError):
+        scoring.token_logprobs(logits, tok)
+    tok[3] = 30
+    scoring.token_logprobs(logits, tok)
+
+
+@pytest.mark.parametrize("at,bad", [((0, 9), 4096), ((0, 1), 5000), ((1, 2), 4096), ((2, 19), -1)],
+                         ids=["scored", "prompt", "masked", "negative"])
+def test_sequences_with_bad_ids_are_refused_before_the_model_runs(scoring, causal_lm, monkeypatch, at, bad):
+    ids, mask = sequences()
+    ids[at] = bad
+    monkeypatch.setattr(causal_lm.model, "forward", lambda *a, **k: pytest.fail("the model ran"))
+    with pytest.raises(ValueError):
+        scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
+
+
+def test_scored_ids_that_the_lm_head_lacks_are_refused(scoring, causal_lm, monkeypatch):
+    """An embedding with more rows than the lm_head (added pad tokens): such ids may stand in the prompt and in masked
+    places, not among the scored tokens."""
+    ids, mask = sequences()
+    monkeypatch.setattr(causal_lm, "lm_head", torch.nn.Linear(256, 4000, bias=False))
+    ids.clamp_(max=3999)
+    ids[0, 2], ids[1, 1] = 4095, 4000
+    mask[2, 17:] = 0
+    ids[2, 18] = 4095
+    scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
+    ids[0, 7] = 4000
+    with pytest.raises(ValueError):
+        scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
