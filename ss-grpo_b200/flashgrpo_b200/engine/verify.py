@@ -169,6 +169,17 @@ class RoundConfig:
     logprobs: int = -1
 
 
+# What a round with log probabilities leaves for a row's pending correction,
+# the next round's root: token, log probability, entropy, alternatives' ids and
+# log probabilities (f32 values by their bits).
+CARRY_WORDS = 3 + 2 * N.FG_MAX_TOPK
+
+
+def carry_fields(carry: torch.Tensor, k: int) -> dict:
+    f, end = carry.view(torch.float32), 3 + N.FG_MAX_TOPK
+    return {"logp": f[:, 1], "entropy": f[:, 2], "top_idx": carry[:, 3:3 + k], "top_logp": f[:, end:end + k]}
+
+
 class DecodeState:
     """Device state of a batch of rollouts between rounds.  max_nodes: with it
     the K/V are an 8-bit cache (`cache`, with lengths q_len / tail_len) that
@@ -196,6 +207,7 @@ class DecodeState:
         self.seq_ids = torch.arange(B, dtype=torch.int32, device=device)
         self.round_dev = torch.zeros(1, dtype=torch.int32, device=device)
         self.X = torch.zeros(((n_heads + 1) * B, spec.hidden), dtype=spec.dtype, device=device)
+        self.carry = torch.full((B, CARRY_WORDS), -1, dtype=torch.int32, device=device)
 
     @property
     def hidden(self) -> torch.Tensor:
@@ -223,6 +235,7 @@ class RoundView:
         self.seq_ids = torch.zeros(B, dtype=torch.int32, device=dev)
         self.round_dev = st.round_dev  # the round counter is shared by all rows
         self.X = torch.zeros(((n_heads + 1) * B, st.X.shape[1]), dtype=st.X.dtype, device=dev)
+        self.carry = torch.full((B, CARRY_WORDS), -1, dtype=torch.int32, device=dev)
         self.k, self.v, self.cache = st.k, st.v, None
         if st.cache is None:
             self.kv_layers = [ops.kv_layer(st.k[l], st.v[l], rows=self.rows) for l in range(st.k.shape[0])]
@@ -236,7 +249,8 @@ class RoundView:
     def hidden(self) -> torch.Tensor:
         return self.X[: self.B]
 
-    def gather(self):
+    def gather(self, carry: bool = False):
+        """The rows' state; carry: of rounds with log probabilities, too."""
         st, idx = self.base, self.rows.long()
         torch.index_select(st.row_len, 0, idx, out=self.row_len)
         torch.index_select(st.pending, 0, idx, out=self.pending)
@@ -246,8 +260,10 @@ class RoundView:
         if self.cache is not None:
             torch.index_select(st.q_len, 0, idx, out=self.q_len)
             torch.index_select(st.tail_len, 0, idx, out=self.tail_len)
+        if carry:
+            torch.index_select(st.carry, 0, idx, out=self.carry)
 
-    def scatter(self):
+    def scatter(self, carry: bool = False):
         st, idx = self.base, self.rows.long()
         st.row_len.index_copy_(0, idx, self.row_len)
         st.pending.index_copy_(0, idx, self.pending)
@@ -256,6 +272,8 @@ class RoundView:
         if self.cache is not None:
             st.q_len.index_copy_(0, idx, self.q_len)
             st.tail_len.index_copy_(0, idx, self.tail_len)
+        if carry:
+            st.carry.index_copy_(0, idx, self.carry)
 
 
 class RoundBuffers:
@@ -380,6 +398,7 @@ class VerifyEngine:
             st.tail_len.zero_()
         st.row_len.zero_()
         st.pending.fill_(-1)
+        st.carry.fill_(-1)
         st.active.fill_(1)
         st.seq_ids.copy_(torch.arange(B, dtype=torch.int32, device=self.device))
         st.round_dev.zero_()
@@ -893,15 +912,17 @@ class VerifyEngine:
         if self.kv8:
             ops.kv8_commit(st.cache, rb.out["acc_nodes"], rb.out["acc_len"], st.q_len, st.tail_len)
         if cfg.logprobs >= 0:
-            self.accepted_logprobs(rb, cfg, B)
+            self.accepted_logprobs(st, rb, cfg)
 
-    def accepted_logprobs(self, rb: RoundBuffers, cfg: RoundConfig, B: int) -> dict:
+    def accepted_logprobs(self, st, rb: RoundBuffers, cfg: RoundConfig) -> dict:
         """Log probability and entropy [B, dcap] of the round's accepted tokens
         under the (tempered) target distribution, and cfg.logprobs
-        alternatives [B, dcap, k]: the root token's from the proposal's root
-        logits, a later path token's from its parent's packed tree logits.
-        Zeros (alternatives -1) behind a row's path."""
-        k, dcap = cfg.logprobs, rb.dcap
+        alternatives [B, dcap, k], each from the logits that the token was
+        drawn from: a root token's are the proposal's root logits or, where it
+        is the correction of the round before, what that round carried; a
+        later path token's, and the new correction's, its parent's packed tree
+        logits.  Zeros (alternatives -1) behind a row's path."""
+        k, dcap, B = cfg.logprobs, rb.dcap, st.B
         bufs = rb.logprobs.get(k)
         if bufs is None:
             f = dict(dtype=torch.float32, device=self.device)
@@ -912,14 +933,22 @@ class VerifyEngine:
             rb.logprobs[k] = bufs
         T = cfg.temperature if cfg.do_sample and cfg.temperature > 0 else 1.0
         tokens, nodes = rb.out["acc_tokens"], rb.out["acc_nodes"]
-        parts = [(slice(0, 1), ops.token_logprobs(rb.logits[:B], tokens[:, 0].contiguous(), temperature=T, k=k))]
+        carried = carry_fields(st.carry, k)
+        r = ops.token_logprobs(rb.logits[:B], tokens[:, 0].contiguous(), temperature=T, k=k)
+        forced = st.carry[:, 0] >= 0
+        for name, buf in bufs.items():
+            new = getattr(r, name)
+            torch.where(forced.view(B, *[1] * (new.dim() - 1)), carried[name], new, out=buf[:, 0])
+        st.carry[:, 0] = st.pending
         if rb.n_int > 0 and dcap > 1:
-            rows = rb.tree["slot"].gather(1, nodes[:, :-1].clamp(min=0).long())
-            parts.append((slice(1, dcap), ops.token_logprobs(rb.tree_logits, tokens[:, 1:].reshape(-1),
-                                                             rows=rows.reshape(-1), temperature=T, k=k)))
-        for cols, r in parts:
+            parents = torch.cat([nodes[:, :-1], rb.out["last_node"][:, None]], 1)
+            rows = rb.tree["slot"].gather(1, parents.clamp(min=0).long())
+            drawn = torch.cat([tokens[:, 1:], st.pending[:, None]], 1)
+            r = ops.token_logprobs(rb.tree_logits, drawn.view(-1), rows=rows.view(-1), temperature=T, k=k)
             for name, buf in bufs.items():
-                buf[:, cols] = getattr(r, name).view(buf[:, cols].shape)
+                new = getattr(r, name).view(buf.shape)
+                buf[:, 1:] = new[:, :-1]
+                carried[name].copy_(new[:, -1])
         return bufs
 
     def view(self, st: DecodeState, B: int, n_heads: int) -> RoundView:
@@ -940,9 +969,9 @@ class VerifyEngine:
         after the proposal and tree build, after the verify forward and the
         internal-node lm_head, and after acceptance + extraction."""
         if isinstance(st, RoundView):
-            st.gather()
+            st.gather(cfg.logprobs >= 0)
             self._round(st, rb, params, cfg, attn_events, phase_events)
-            st.scatter()
+            st.scatter(cfg.logprobs >= 0)
         else:
             self._round(st, rb, params, cfg, attn_events, phase_events)
 

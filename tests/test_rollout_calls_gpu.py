@@ -98,3 +98,53 @@ def test_sequence_logprobs_memory_goes_by_the_chunk():
     assert held[256] + 56 * mb < held[4096], held
     assert peak[256] < held[256] + 32 * mb < peak[4096], (held, peak)
     assert (grads[256] - grads[4096]).norm() <= 2.5e-4 * grads[4096].norm()
+
+
+@pytest.mark.parametrize("k,sample", [(0, True), (3, True), (2, False)])
+def test_a_correction_keeps_the_log_probabilities_of_its_draw(bf16_model, monkeypatch, k, sample):
+    """A round's correction is the next round's root.  What is reported for it is what its parent's tree logits say in
+    the round that drew it, bit for bit, whatever the next proposal's own GEMM and rounding make of the same hidden
+    state; rows that finish earlier leave the batch in between."""
+    from flashgrpo_b200 import _native, ops
+    from flashgrpo_b200.engine.verify import VerifyEngine
+    from flashgrpo_b200.utils import synthetic
+
+    dec = bf16_decoder(bf16_model, return_logprobs=True, logprob_alternatives=k, use_cuda_graphs=False,
+                       do_sample=sample, temperature=0.8 if sample else 1.0)
+    T = 0.8 if sample else 1.0
+    want, seen, sizes = {}, [0], set()
+    inner = VerifyEngine.accept
+
+    def accept(self, st, rb, cfg, phase_event=None):
+        inner(self, st, rb, cfg, phase_event=phase_event)
+        names = ["logp", "entropy"] + (["top_idx", "top_logp"] if k else [])
+        here = st.rows.tolist() if hasattr(st, "rows") else list(range(st.B))
+        sizes.add(st.B)
+        for i, row in enumerate(here):
+            if row in want:
+                seen[0] += 1
+                tok, vals = want.pop(row)
+                assert int(rb.out["acc_tokens"][i, 0]) == tok
+                for name in names:
+                    assert torch.equal(rb.logprobs[k][name][i, 0], vals[name]), (row, name)
+            if int(st.pending[i]) >= 0:
+                at = rb.tree["slot"][i, int(rb.out["last_node"][i])].view(1)
+                r = ops.token_logprobs(rb.tree_logits, st.pending[i:i + 1].contiguous(), rows=at.contiguous(),
+                                       temperature=T, k=k)
+                want[row] = int(st.pending[i]), {n: getattr(r, n)[0].clone() for n in names}
+
+    monkeypatch.setattr(VerifyEngine, "accept", accept)
+    ids, mask = synthetic.random_prompts(3, 40, 4096, seed=8)
+    mask[0, :9], mask[2, :30] = 0, 0
+    res = dec.generate(ids, mask, repeated_generate_nums=2, max_length=60)
+    monkeypatch.undo()
+    assert seen[0] > 40 and len(sizes) > 1
+    # captured rounds, twice on one decoder: the same values
+    dec = bf16_decoder(bf16_model, return_logprobs=True, logprob_alternatives=k, do_sample=sample,
+                       temperature=0.8 if sample else 1.0)
+    for _ in range(2):
+        again = dec.generate(ids, mask, repeated_generate_nums=2, max_length=60)
+        for key in ("generated_token_ids", "generated_logprobs", "generated_entropies"):
+            assert again[key] == res[key]
+        assert again.get("generated_alternatives") == res.get("generated_alternatives")
+    assert _native.read_device_error(clear=True) == 0
