@@ -123,6 +123,8 @@ class FlashMedusaDecoder:
             raise ValueError(f"Unsupported kv_cache_dtype={config.kv_cache_dtype}")
         if not 0 <= int(config.logprob_alternatives) <= 16:
             raise ValueError("logprob_alternatives must be between 0 and 16")
+        if config.logprob_alternatives and not config.return_logprobs:
+            raise ValueError("logprob_alternatives needs return_logprobs")
         self._engine: VerifyEngine | None = None
         # captured round graphs, keyed by (state, round shape, round config);
         # a shape is run eagerly once before it is captured

@@ -194,3 +194,11 @@ def test_scored_ids_that_the_lm_head_lacks_are_refused(scoring, causal_lm, monke
     ids[0, 7] = 4000
     with pytest.raises(ValueError):
         scoring.sequence_logprobs(causal_lm, ids, mask, prompt_len=5)
+
+
+def test_alternatives_without_log_probabilities_are_refused():
+    from flashgrpo_b200.decoding.flash_medusa_decoder import FlashMedusaConfig, FlashMedusaDecoder
+
+    with pytest.raises(ValueError):
+        FlashMedusaDecoder(None, None, None, FlashMedusaConfig(logprob_alternatives=3))
+    FlashMedusaDecoder(None, None, None, FlashMedusaConfig(logprob_alternatives=3, return_logprobs=True))
