@@ -50,6 +50,13 @@ def _need(t: torch.Tensor, name: str, dtype=None, contiguous=True):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _on(device: torch.device, **tensors):
+    """All on one device: a kernel that is given another GPU's memory faults."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call on {device}")
+
+
 def _out(t: torch.Tensor, name: str, dtype, n: int):
     """An output the kernel writes as n contiguous elements of dtype."""
     if t.dtype != dtype or not t.is_contiguous() or t.numel() < n:
@@ -167,6 +174,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, rows: torch.Te
         if k:
             _out(out.top_idx, "top_idx", torch.int32, n * k)
             _out(out.top_logp, "top_logp", torch.float32, n * k)
+        _on(logits.device, **{name: getattr(out, name) for name in out._fields[:5 if k else 3]})
     _call(logits, "fg_token_logprobs", _ptr(logits), dtype_code(logits), stride, vocab, logits.shape[0], _ptr(rows),
            _ptr(tokens), n, float(temperature), _ptr(out.logp), _ptr(out.entropy), _ptr(out.lse), k,
            _ptr(out.top_idx), _ptr(out.top_logp), _stream(logits))
@@ -196,6 +204,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, lse: tor
     ostride, ov = _rows(out, "out")
     if ov != vocab or out.shape[0] < n:
         raise ValueError("out must have the logits' shape")
+    _on(logits.device, lse=lse, entropy=entropy, grad_logp=grad_logp, grad_entropy=grad_entropy, out=out)
     _call(logits, "fg_token_logprobs_backward", _ptr(logits), dtype_code(logits), stride, vocab, _ptr(tokens), n,
            float(temperature), _ptr(lse), _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(out), ostride,
            _stream(logits))
@@ -534,6 +543,7 @@ def kv8_load(cache: Kv8Cache, layer: int, k: torch.Tensor, v: torch.Tensor, leng
     _need(lengths, "lengths", torch.int32)
     if lengths.shape != (P,):
         raise ValueError(f"lengths must be [{P}]")
+    _on(cache.device, v=v, lengths=lengths)
     cache._lengths(q_len, tail_len, P * int(repeats))
     _call(k, "fg_kv8_load", cache._ref, int(layer), _ptr(k), _ptr(v), k.stride(0), k.stride(1), k.stride(2), k.shape[2],
            _ptr(lengths), P, int(repeats), _ptr(q_len), _ptr(tail_len), _stream(k))
@@ -553,6 +563,7 @@ def kv8_commit(cache: Kv8Cache, acc_nodes: torch.Tensor, acc_len: torch.Tensor, 
     B = acc_len.shape[0]
     if acc_nodes.dim() != 2 or acc_nodes.shape[0] != B:
         raise ValueError("acc_nodes must be [B, dcap]")
+    _on(cache.device, acc_nodes=acc_nodes, acc_len=acc_len)
     cache._lengths(q_len, tail_len, B)
     if (q_len_out is None) != (tail_len_out is None):
         raise ValueError("q_len_out and tail_len_out go together")
@@ -595,6 +606,7 @@ def tree_attention_kv8(q: torch.Tensor, cache: Kv8Cache, layer: int, q_len: torc
     if workspace is not None:
         _need(workspace, "workspace")
         ws_bytes = workspace.numel() * workspace.element_size()
+    _on(cache.device, anc=anc, out=out, workspace=workspace)
     _call(q, "fg_tree_attention_kv8", _ptr(q), cache._ref, int(layer), _ptr(q_len), _ptr(tail_len), _ptr(anc), B,
            n_nodes, hq, float(scale), _ptr(out), _ptr(workspace), ws_bytes, int(num_splits),
            cache.capacity if max_q_len is None else int(max_q_len), _stream(q))

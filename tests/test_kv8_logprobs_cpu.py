@@ -124,3 +124,71 @@ def test_decoder_options():
     for bad in (dict(kv_cache_dtype="int8"), dict(logprob_alternatives=17), dict(logprob_alternatives=-1)):
         with pytest.raises(ValueError):
             FlashMedusaDecoder(None, None, None, FlashMedusaConfig(**bad))
+
+
+# ------------------------------------------------------ tensors of two devices
+@pytest.fixture
+def fake(monkeypatch):
+    """The wrappers over tensors without memory (so of any device); the calls that pass their checks are listed."""
+    from flashgrpo_b200 import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    called = []
+    monkeypatch.setattr(ops, "_ptr", lambda t: None if t is None else 1 << 20)
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+    monkeypatch.setattr(ops, "_call", lambda t, name, *a, **k: called.append(name))
+    with FakeTensorMode():
+        yield ops, called
+
+
+def two_devices(call, args, called, name):
+    """call(**args) on one device runs; with any one tensor on another it is refused before the launch."""
+    import torch
+
+    call(**args)
+    assert called == [name]
+    for key, t in args.items():
+        if isinstance(t, torch.Tensor):
+            with pytest.raises(ValueError):
+                call(**{**args, key: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="cuda:1")})
+    assert called == [name]
+
+
+def test_cache_calls_with_tensors_of_two_devices(fake):
+    import torch
+
+    ops, called = fake
+    on = dict(device="cuda:0")
+    i32 = lambda *s: torch.empty(s, dtype=torch.int32, **on)  # noqa: E731
+    cache = ops.Kv8Cache.empty(1, 2, 2, 64, 128, max_nodes=8, dtype=torch.bfloat16, **on)
+    kv = dict(dtype=torch.bfloat16, **on)
+    two_devices(lambda **a: ops.kv8_load(cache, 0, **a),
+                dict(k=torch.empty(2, 2, 40, 128, **kv), v=torch.empty(2, 2, 40, 128, **kv), lengths=i32(2),
+                     q_len=i32(2), tail_len=i32(2)), called, "fg_kv8_load")
+    called.clear()
+    two_devices(lambda **a: ops.kv8_commit(cache, **a),
+                dict(acc_nodes=i32(2, 4), acc_len=i32(2), q_len=i32(2), tail_len=i32(2), q_len_out=i32(2),
+                     tail_len_out=i32(2)), called, "fg_kv8_commit")
+    called.clear()
+    q = torch.empty(2, 8, 4, 128, **kv)
+    two_devices(lambda **a: ops.tree_attention_kv8(cache=cache, layer=0, scale=1.0, **a),
+                dict(q=q, q_len=i32(2), tail_len=i32(2), anc=i32(8, 4), out=torch.empty_like(q), workspace=i32(64)),
+                called, "fg_tree_attention_kv8")
+
+
+def test_logprob_calls_with_tensors_of_two_devices(fake):
+    import torch
+
+    ops, called = fake
+    on = dict(device="cuda:0")
+    f = lambda *s: torch.empty(s, **on)  # noqa: E731
+    i32 = lambda *s: torch.empty(s, dtype=torch.int32, **on)  # noqa: E731
+    names = ops.TokenLogprobs._fields
+    two_devices(lambda logits, tokens, rows, **o: ops.token_logprobs(logits, tokens, rows=rows, k=2,
+                                                                     out=ops.TokenLogprobs(**o)),
+                dict(logits=f(4, 50), tokens=i32(4), rows=i32(4),
+                     **dict(zip(names, (f(4), f(4), f(4), i32(4, 2), f(4, 2))))), called, "fg_token_logprobs")
+    called.clear()
+    two_devices(ops.token_logprobs_backward,
+                dict(logits=f(4, 50), tokens=i32(4), lse=f(4), entropy=f(4), grad_logp=f(4), grad_entropy=f(4),
+                     out=f(4, 50)), called, "fg_token_logprobs_backward")
