@@ -401,7 +401,8 @@ typedef struct fg_kv8_cache {
  * [n_src * repeats] get the rows' lengths.  Other slots keep what they hold.
  * src_len / FG_KV8_BLOCK whole blocks must fit the capacity (FG_ECAPACITY); a
  * length outside [0, src_len] or a mapped row outside the cache records
- * FG_EINVAL in the device error word and loads nothing (lengths 0). */
+ * FG_EINVAL in the device error word and loads nothing (lengths 0).  q_len and
+ * tail_len share no memory with each other, lengths or the row map (FG_EINVAL). */
 fg_status fg_kv8_load(const fg_kv8_cache *cache, int32_t layer, const void *k, const void *v, int64_t stride_b,
                       int64_t stride_h, int64_t stride_s, int32_t src_len, const int32_t *lengths, int32_t n_src,
                       int32_t repeats, int32_t *q_len, int32_t *tail_len, void *stream);
@@ -416,7 +417,8 @@ fg_status fg_kv8_load(const fg_kv8_cache *cache, int32_t layer, const void *k, c
  * NULL or the inputs themselves: in place, by a second small kernel).  A row whose lengths,
  * path or mapped row do not fit the cache (FG_EINVAL in the device error
  * word) or whose block does not fit the capacity (FG_ECAPACITY there) stays
- * as it is, its lengths too. */
+ * as it is, its lengths too.  The lengths written share no memory with each
+ * other or with the other inputs (FG_EINVAL). */
 fg_status fg_kv8_commit(const fg_kv8_cache *cache, const int32_t *acc_nodes, int32_t dcap, const int32_t *acc_len,
                         int32_t B, int32_t *q_len, int32_t *tail_len, int32_t *q_len_out, int32_t *tail_len_out,
                         void *stream);

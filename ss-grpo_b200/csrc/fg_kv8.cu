@@ -337,6 +337,12 @@ static fg_status check_cache(const fg_kv8_cache* c, int32_t B) {
     return FG_OK;
 }
 
+// Whether two int32 arrays share memory (NULL shares with none): lengths that
+// a kernel writes while other CTAs still read them as something else.
+static bool overlap(const int32_t* a, int64_t na, const int32_t* b, int64_t nb) {
+    return a && b && (uintptr_t)a < (uintptr_t)(b + nb) && (uintptr_t)b < (uintptr_t)(a + na);
+}
+
 }  // namespace kv8
 }  // namespace fg
 
@@ -354,6 +360,10 @@ extern "C" fg_status fg_kv8_load(const fg_kv8_cache* cache, int32_t layer, const
         !tail_len || q_len == tail_len)
         return FG_EINVAL;
     if (src_len / kv8::kBlk * kv8::kBlk > cache->capacity) return FG_ECAPACITY;
+    const int64_t n = (int64_t)n_src * repeats;
+    if (kv8::overlap(q_len, n, tail_len, n)) return FG_EINVAL;
+    for (const int32_t* out : {q_len, tail_len})
+        if (kv8::overlap(out, n, lengths, n_src) || kv8::overlap(out, n, cache->rows, n)) return FG_EINVAL;
     const int esz = cache->dtype == FG_DTYPE_F32 ? 4 : 2;
     const bool vec = (((uintptr_t)k | (uintptr_t)v) % 16 == 0) && (stride_b * esz) % 16 == 0 &&
                      (stride_h * esz) % 16 == 0 && (stride_s * esz) % 16 == 0;
@@ -381,10 +391,14 @@ extern "C" fg_status fg_kv8_commit(const fg_kv8_cache* cache, const int32_t* acc
     if (!acc_nodes || !acc_len || !q_len || !tail_len || q_len == tail_len || dcap <= 0 || !q_len_out != !tail_len_out) return FG_EINVAL;
     if (dcap > FG_MAX_PATH) return FG_ECAPACITY;
     if (q_len_out == q_len && tail_len_out == tail_len) q_len_out = tail_len_out = nullptr;  // in place
-    // lengths that some CTAs still read must not change under them
-    if (q_len_out && (q_len_out == q_len || q_len_out == tail_len || tail_len_out == q_len ||
-                      tail_len_out == tail_len || q_len_out == tail_len_out))
-        return FG_EINVAL;
+    // lengths, paths and rows that some CTAs still read must not change under them
+    if (kv8::overlap(q_len, B, tail_len, B) || kv8::overlap(q_len_out, B, tail_len_out, B)) return FG_EINVAL;
+    for (const int32_t* out : {q_len_out, tail_len_out})
+        if (kv8::overlap(out, B, q_len, B) || kv8::overlap(out, B, tail_len, B)) return FG_EINVAL;
+    for (const int32_t* out : {q_len_out ? q_len_out : q_len, q_len_out ? tail_len_out : tail_len})
+        if (kv8::overlap(out, B, acc_len, B) || kv8::overlap(out, B, acc_nodes, (int64_t)B * dcap) ||
+            kv8::overlap(out, B, cache->rows, B))
+            return FG_EINVAL;
     const dim3 grid(2 * cache->n_kv_heads, cache->n_layers, B);
     cudaStream_t st = (cudaStream_t)stream;
     if (cache->dtype == FG_DTYPE_F32)

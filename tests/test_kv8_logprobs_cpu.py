@@ -192,3 +192,24 @@ def test_logprob_calls_with_tensors_of_two_devices(fake):
     two_devices(ops.token_logprobs_backward,
                 dict(logits=f(4, 50), tokens=i32(4), lse=f(4), entropy=f(4), grad_logp=f(4), grad_entropy=f(4),
                      out=f(4, 50)), called, "fg_token_logprobs_backward")
+
+
+# ------------------------------------------------ lengths that share memory
+@pytest.mark.parametrize("lens,q,t,rows", [(0, 0, 64, None), (0, 64, 0, None), (0, 64, 12, None), (0, -12, 64, None),
+                                           (0, 64, 72, None), (0, 64, 128, 64), (0, 64, 128, 140)])
+def test_load_lengths_that_share_memory(N, lens, q, t, rows):
+    """A CTA writes a row's lengths while others still read the source's."""
+    lib, at = N.load(), lambda off: None if off is None else ctypes.c_void_p((1 << 22) + off)  # noqa: E731
+    c = cache(N, rows=None if rows is None else (1 << 22) + rows)
+    assert lib.fg_kv8_load(c, 0, P, P, 128, 128, 128, 33, at(lens), 4, 1, at(q), at(t), None) == N.FG_EINVAL
+
+
+@pytest.mark.parametrize("nodes,acc,q,t,qo,to,rows", [
+    (0, 64, 64, 128, None, None, None), (0, 64, 128, 64, None, None, None), (0, 128, 60, 192, None, None, None),
+    (0, 128, 192, 200, None, None, None), (0, 128, 192, 256, None, None, 192), (0, 128, 192, 256, None, None, 250),
+    (0, 128, 192, 256, 128, 320, None), (0, 128, 192, 256, 320, 48, None), (0, 128, 192, 256, 320, 332, None),
+    (0, 128, 192, 256, 196, 320, None), (0, 128, 192, 256, 320, 384, 384)])
+def test_commit_lengths_that_share_memory(N, nodes, acc, q, t, qo, to, rows):
+    lib, at = N.load(), lambda off: None if off is None else ctypes.c_void_p((1 << 22) + off)  # noqa: E731
+    c = cache(N, rows=None if rows is None else (1 << 22) + rows)
+    assert lib.fg_kv8_commit(c, at(nodes), 4, at(acc), 4, at(q), at(t), at(qo), at(to), None) == N.FG_EINVAL
