@@ -148,3 +148,19 @@ def test_a_correction_keeps_the_log_probabilities_of_its_draw(bf16_model, monkey
             assert again[key] == res[key]
         assert again.get("generated_alternatives") == res.get("generated_alternatives")
     assert _native.read_device_error(clear=True) == 0
+
+
+def test_one_decoder_with_two_batches(bf16_model):
+    """One row, many rows, one row: the proposal's workspace grows in between, and the captured rounds of the small
+    batch are replayed behind it."""
+    from flashgrpo_b200 import _native
+    from flashgrpo_b200.utils import synthetic
+
+    dec = bf16_decoder(bf16_model, return_logprobs=True)
+    ids, mask = synthetic.random_prompts(1, 20, 4096, seed=3)
+    got = {1: [], 48: []}
+    for n in (1, 1, 48, 48, 1, 48, 1):
+        r = dec.generate(ids, mask, repeated_generate_nums=n, max_length=44)
+        got[n].append((r["generated_token_ids"], r["generated_logprobs"]))
+    assert all(x == got[1][0] for x in got[1]) and all(x == got[48][0] for x in got[48])
+    assert _native.read_device_error(clear=True) == 0
