@@ -137,8 +137,8 @@ fg_status fg_row_topk(const void *logits, int32_t dtype, int64_t row_stride, int
  * (its alternatives are chosen among the entries that are not NaN; index -1
  * where there are fewer than k).  A padded entry (token < 0) gets zeros and
  * alternatives -1; so does a token >= vocab or a row outside [0, n_rows),
- * which records FG_EINVAL in the device error word.  temperature > 0 and
- * finite.  The whole (tempered) distribution is meant, without a nucleus or
+ * which records FG_EINVAL in the device error word.  temperature > 0, it and
+ * log2 e / temperature finite.  The whole (tempered) distribution is meant, without a nucleus or
  * top-k cut.  Replaces the reference trainer's log-softmax + gather. */
 fg_status fg_token_logprobs(const void *logits, int32_t dtype, int64_t row_stride, int32_t vocab, int32_t n_rows,
                             const int32_t *rows, const int32_t *tokens, int32_t n, float temperature, float *logp,

@@ -565,11 +565,19 @@ __global__ void __launch_bounds__(kBT) logprobs_backward_kernel(const BwdParams 
 }
 
 // Rows up to kShort vectors take one 128-thread CTA each; longer ones 512
-// threads, and a cluster of CTAs per row while there are fewer of them than
-// SMs (192 rows of 151936 with four alternatives: clusters of 8 / 4 / 2 / 1
-// take 65 / 41 / 33 / 31 us; the largest batch, 4096 rows, streams at 0.88 of
-// the copy bandwidth, 219 us).
+// threads, and a cluster of CTAs per row while all of them fit on the SMs at
+// once: eight up to 18 rows, two up to 74, one from there on (151936 bf16
+// logits with four alternatives, us at 8 / 2 / 1 CTAs a row: 8 rows 12.4 / 15.1
+// / 20.0, 18 rows 14.4 / 15.1 / 20.6, 37 rows 22.4 / 15.1 / 20.6, 74 rows 32.8
+// / 15.8 / 21.3, 192 rows 70.6 / 35.6 / 32.2).  Four are not used: 13.1 at 18
+// and 30 rows, 16.0 at 37; two would still be faster at 110 rows, 21.0 against
+// 24.0.  The largest batch, 4096 rows, streams at 0.88 of the copy bandwidth,
+// 220 us.
 constexpr int kShort = 1024;
+
+// The kernels multiply by log2 e / T: a T so small that this is infinite makes
+// NaN of the maximum's 0.
+static bool good_temperature(float t) { return t > 0.0f && t < INFINITY && kLog2e / t < INFINITY; }
 
 template <typename T, int NT, int CL>
 static cudaError_t launch_fwd(const FwdParams& p, cudaStream_t st) {
@@ -619,7 +627,7 @@ extern "C" fg_status fg_token_logprobs(const void* logits, int32_t dtype, int64_
                                        int32_t* top_idx, float* top_logp, void* stream) {
     if (n == 0) return FG_OK;
     if (!logits || !tokens || !logp || n < 0 || vocab <= 0 || n_rows <= 0 || (row_stride < vocab && n_rows > 1) ||
-        (!rows && n_rows < n) || !(temperature > 0.0f) || !(temperature < INFINITY) || k < 0)
+        (!rows && n_rows < n) || !lp::good_temperature(temperature) || k < 0)
         return FG_EINVAL;
     if (dtype != FG_DTYPE_F32 && dtype != FG_DTYPE_BF16 && dtype != FG_DTYPE_F16) return FG_EINVAL;
     if (k > FG_MAX_TOPK || k > vocab) return FG_ECAPACITY;
@@ -644,8 +652,8 @@ extern "C" fg_status fg_token_logprobs_backward(const void* logits, int32_t dtyp
                                                 void* stream) {
     if (n == 0) return FG_OK;
     if (!logits || !tokens || !lse || !grad_logp || !grad_logits || n < 0 || vocab <= 0 ||
-        (n > 1 && (row_stride < vocab || grad_stride < vocab)) || !(temperature > 0.0f) ||
-        !(temperature < INFINITY) || (grad_entropy && !entropy))
+        (n > 1 && (row_stride < vocab || grad_stride < vocab)) || !lp::good_temperature(temperature) ||
+        (grad_entropy && !entropy))
         return FG_EINVAL;
     if (dtype != FG_DTYPE_F32 && dtype != FG_DTYPE_BF16 && dtype != FG_DTYPE_F16) return FG_EINVAL;
     // in place means the same rows at the same places; any other overlap is a race

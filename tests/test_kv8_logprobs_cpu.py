@@ -213,3 +213,11 @@ def test_commit_lengths_that_share_memory(N, nodes, acc, q, t, qo, to, rows):
     lib, at = N.load(), lambda off: None if off is None else ctypes.c_void_p((1 << 22) + off)  # noqa: E731
     c = cache(N, rows=None if rows is None else (1 << 22) + rows)
     assert lib.fg_kv8_commit(c, at(nodes), 4, at(acc), 4, at(q), at(t), at(qo), at(to), None) == N.FG_EINVAL
+
+
+@pytest.mark.parametrize("T", [1e-45, 1e-40, 4.2e-39])
+def test_temperatures_without_a_finite_reciprocal(N, T):
+    """log2 e / T is infinite in fp32: every row's maximum would become NaN."""
+    lib, far = N.load(), ctypes.c_void_p(1 << 30)
+    assert lib.fg_token_logprobs(P, 1, 100, 100, 8, None, P, 8, T, P, P, P, 0, P, P, None) == N.FG_EINVAL
+    assert lib.fg_token_logprobs_backward(P, 1, 100, 100, P, 8, T, P, P, P, P, far, 100, None) == N.FG_EINVAL
