@@ -47,13 +47,17 @@
 //
 // What bounds it: neither HBM nor the tensor pipe (8 MMAs take 380-530 clocks
 // of a tile's ~2500) but the softmax warps' chain of TMEM load, vote,
-// exponentials and stores per tile.  Measured steps at 64 query rows, 32 rows
-// x 8 heads x 16384 slots (1.09 GB, 168 us at the copy bandwidth): K and V
-// widened to bf16 from register prefetches 636 us (a release on a barrier
-// waits for the loads a thread has in flight, so they hid nothing), TMA
-// staging and scales in shared memory 360 us, plain try_wait 349 us, maxima by
-// one redux each 344 us; the bf16 kernel on a bf16 cache of twice the bytes
-// takes 360 us.
+// exponentials and stores per tile.  Measured at 64 query rows, 32 rows x 8
+// heads x 16384 slots (1.09 GB, 168 us at the copy bandwidth): 354 us on keys
+// with strong channels; the bf16 kernel on a bf16 cache of the same values
+// (twice the bytes) 335 us.  The steps to it, on uniform codes, whose maxima
+// hardly call for new references: K and V widened to bf16 from register
+// prefetches 636 us (a release on a barrier waits for the loads a thread has in
+// flight, so they hid nothing), TMA staging and scales in shared memory 360 us,
+// plain try_wait 349 us, maxima by one redux each 344 us.  With more query rows
+// per head the bf16 kernel is the faster one: 78 rows, 64 x 1024: 42.6 against
+// 19.9 us; 224 rows, 16 x 2048: 65.4 against 30.8; with one node this one is:
+// 254 against 329 us at 32 x 16384.
 #include "fg_common.cuh"
 
 namespace fg {
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_kv8_tc_kernel(const __grid
     static_assert(3 * R2 <= (int)kCols, "TMEM columns");
     // registers: 128 a thread at launch, 512 per lane slot of the four warps
     // of a scheduler; the softmax keeps H sums.  (A spilled register costs a trip to L2: the streams leave
-    // nothing of the little L1.)
+    // nothing of the little L1.  The forms for more than 32 query rows spill 12 bytes and load 76 to 84.)
     constexpr int kRegSoft = 176, kRegConv = 96, kRegMma = 64;
     static_assert(2 * kRegSoft + kRegConv + kRegMma <= 512, "register split");
     constexpr int kKStages = Smem<NC>::kKStages, kOffVRing = Smem<NC>::kOffV, kOffPBuf = Smem<NC>::kOffP;

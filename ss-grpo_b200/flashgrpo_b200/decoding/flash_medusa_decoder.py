@@ -86,7 +86,8 @@ class FlashMedusaConfig:
     dense_kernel: str = "auto"
     autotune_dense: bool = True    # time fg_linear's tilings once per projection shape
     # K/V of finished blocks of 32 tokens: "model" (the model's dtype) or "fp8" (e4m3 with a scale per block and
-    # head: half the bytes; the newest tokens and the tree stay in the model's dtype)
+    # head: half the bytes, at up to twice the attention time with trees; the newest tokens and the tree stay in the
+    # model's dtype)
     kv_cache_dtype: str = "model"
     # log probability and entropy of every generated token under the distribution it was drawn from (before a
     # top_p / top_k cut), as "generated_logprobs" / "generated_entropies", and so many best alternatives
