@@ -80,8 +80,8 @@ def sequence_logprobs(causal_lm, input_ids: torch.Tensor, attention_mask: torch.
         raise ValueError("attention_mask must have the shape of input_ids")
     base = unwrap_causal_lm(causal_lm)
     _check_ids(input_ids, 0, base.model.get_input_embeddings().weight.shape[0], "input_ids")
-    _check_ids(torch.where(attention_mask.to(input_ids.device) > 0, input_ids, 0)[:, prompt_len:], 0, base.lm_head.weight.shape[0],
-               "scored input_ids")
+    scored = torch.where(attention_mask.to(input_ids.device) > 0, input_ids, 0)[:, prompt_len:]
+    _check_ids(scored, 0, base.lm_head.weight.shape[0], "scored input_ids")
     dev = base.lm_head.weight.device
     ids, mask = input_ids.to(dev), attention_mask.to(dev).long()
     pos = (mask.cumsum(-1) - 1).clamp(min=0)
